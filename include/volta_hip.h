@@ -453,7 +453,7 @@ int vh_residual_norm(int dtype, const void* x, const void* block, const void* ga
                      int64_t gate_rows, float scale, float eps, void* stream);
 /* Its backward, from grad_y (NULL: nothing but n uses y) and grad_n (with next_weight):
  * grad_x and grad_block, and the gradient of every gate and weight that is given, summed
- * over the rows that share it in a fixed order.  x, block and rstd are the forward's.
+ * over the rows that share it in a fixed order (0 where there are no rows).  x, block and rstd are the forward's.
  * grad_x may be grad_y, grad_block may be grad_n or block. */
 int vh_residual_norm_backward(int dtype, const void* grad_y, const void* grad_n, const void* x, const void* block,
                               const float* rstd, const void* gate, const void* post_weight, const void* next_weight,

@@ -252,3 +252,34 @@ def test_refuses_more_rows_than_a_launch_has_threads():
     assert _lib.lib().vh_residual_norm(0, x, x, None, None, None, x, None, r.data_ptr(), rows, 8, 0, 1.0, 1e-6, s) == _lib.VH_ERR_UNSUPPORTED
     assert _lib.lib().vh_residual_norm_backward(0, x, None, x, x, r.data_ptr(), None, None, None, x, x, None, None, None, rows, 8, 0, 1.0,
                                                 s) == _lib.VH_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_rows_leave_the_gate_no_gradient(dtype):
+    """The sum over no rows is 0, whatever the buffer held: for weights and gates alike."""
+    lib, s, dt = _lib.lib(), ops.stream_ptr(torch.device(DEV)), ops.dtype_code(torch.empty(0, dtype=dtype))
+    E, width = _lib, 72
+    one = torch.ones(width, dtype=dtype, device=DEV).data_ptr()
+
+    def call(gate_rows, grad_gate):
+        gate = torch.ones((max(gate_rows, 1), width), dtype=dtype, device=DEV)
+        sums = [torch.full((width,), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+        status = lib.vh_residual_norm_backward(dt, None, None, None, None, None, gate.data_ptr(), one, one, None, None,
+                                               grad_gate, sums[0].data_ptr(), sums[1].data_ptr(), 0, width, gate_rows, 1.0, s)
+        return status, sums
+
+    for gate_rows in (1, 5):
+        held = torch.full((gate_rows + 1, width), 7.0, dtype=dtype, device=DEV)
+        status, sums = call(gate_rows, held.data_ptr())
+        assert status == E.VH_OK and not held[:gate_rows].any() and bool((held[gate_rows:] == 7).all())
+        assert not sums[0].any() and not sums[1].any()
+    assert call(1, None)[0] == E.VH_ERR_BAD_ARG
+    assert call(-1, one)[0] == E.VH_ERR_BAD_SHAPE
+    assert call(0, None)[0] == E.VH_OK  # a gate row for each of no rows
+    t = make(0, width, dtype, 1)
+    y, n, rstd = ops.gpu_residual_norm(t["x"], t["b"], t["gate"], t["wp"], t["wn"])
+    del one
+    junk = torch.full((1, width), 7.0, dtype=dtype, device=DEV)
+    del junk  # the next allocation of this size
+    dgate = ops.gpu_residual_norm_backward(t["dy"], t["dn"], t["x"], t["b"], rstd, t["gate"], t["wp"], t["wn"])[2]
+    assert dgate.shape == (1, width) and not dgate.any()

@@ -1957,8 +1957,12 @@ static int check_norm(int dtype, const void* gate, int64_t rows, int64_t width, 
   if (width > kNormMostWidth) return set_error(VH_ERR_UNSUPPORTED, "rows of %ld elements: at most %ld", (long)width, kNormMostWidth);
   if (rows > (1L << 26) - 16) return set_error(VH_ERR_UNSUPPORTED, "%ld rows", (long)rows);  // 64 threads or more each, of 2^32
   VH_TRY(check_sizes({(long)(rows * width)}));
-  if (gate && rows && (gate_rows <= 0 || rows % gate_rows))
+  if (gate && (gate_rows < (rows ? 1 : 0) || (rows && rows % gate_rows)))
     return set_error(VH_ERR_BAD_SHAPE, "%ld gate rows do not divide %ld rows", (long)gate_rows, (long)rows);
+  if (gate && !rows) {  // gate rows that no row has
+    if (gate_rows > (1L << 26) - 16) return set_error(VH_ERR_UNSUPPORTED, "%ld gate rows", (long)gate_rows);
+    VH_TRY(check_sizes({(long)(gate_rows * width)}));
+  }
   return VH_OK;
 }
 
@@ -1982,9 +1986,10 @@ int vh_residual_norm_backward(int dtype, const void* grad_y, const void* grad_n,
   VH_ENTRY();
   VH_TRY(check_norm(dtype, gate, rows, width, gate_rows));
   hipStream_t st = S(stream);
-  if ((gate && !grad_gate && rows) || (post_weight && !grad_post_weight) || (next_weight && !grad_next_weight))
+  if ((gate && !grad_gate && gate_rows) || (post_weight && !grad_post_weight) || (next_weight && !grad_next_weight))
     return set_error(VH_ERR_BAD_ARG, "null pointer");
   if (rows == 0) {  // sums of nothing
+    if (gate && gate_rows) VH_TRY(VH_DISPATCH(dtype, run_fill, grad_gate, (long)(gate_rows * width), 0.f, st));
     if (post_weight) VH_TRY(VH_DISPATCH(dtype, run_fill, grad_post_weight, (long)width, 0.f, st));
     if (next_weight) VH_TRY(VH_DISPATCH(dtype, run_fill, grad_next_weight, (long)width, 0.f, st));
     return VH_OK;
