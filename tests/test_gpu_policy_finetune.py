@@ -75,3 +75,27 @@ def test_muon_takes_kernels():
     m = torch.zeros_like(flat)
     volta_amd.ops.gpu_muon_step(flat, dw.reshape(24, -1), m, 0.1, nesterov=False)
     assert torch.equal(w.reshape(24, -1), flat) and torch.equal(opt.momentum[0].reshape(24, -1), m)
+
+
+def test_muon_refuses_before_it_updates():
+    """A gradient of another shape (a transposed one has as many elements), type or layout, wherever in the list:
+    no parameter and no momentum has changed."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    n = lambda *s: torch.randn(s, generator=g, device=DEV)  # noqa: E731
+    params = [n(48, 32), n(24, 6, 3, 3), n(784, 512)]
+    good = [n(*p.shape) for p in params]
+    E = volta_amd.VoltaHipError
+    bad = ((0, n(32, 48), E), (1, n(6, 24, 3, 3), E), (1, n(54, 24), E), (2, n(512, 784), E), (2, n(784 * 512), E),
+           (2, n(784, 512).bfloat16(), TypeError), (2, n(512, 784).t(), ValueError),
+           (1, n(24, 6, 3, 3).to(memory_format=torch.channels_last), ValueError), (2, n(784, 512).cpu(), E), (2, None, TypeError))
+    for at, wrong, kind in bad:
+        opt = nn.Muon(params, lr=0.1)
+        before = [t.clone() for t in params + opt.momentum]
+        grads = list(good)
+        grads[at] = wrong
+        with pytest.raises(kind):
+            opt.step(grads)
+        assert all(torch.equal(a, b) for a, b in zip(params + opt.momentum, before))
+    good[1] = good[1].view(24, 54)  # a kernel's matrix
+    opt.step(good)
+    assert not any(torch.equal(a, b) for a, b in zip(params + opt.momentum, before))

@@ -370,9 +370,23 @@ class Muon:
         self.nesterov, self.steps, self.eps = nesterov, steps, eps
 
     def step(self, grads) -> None:
+        """Every gradient has its parameter's shape (or that of its matrix), dtype and device, and is contiguous:
+        checked for all of them before the first update."""
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"Muon: {len(grads)} gradients for {len(self.params)} parameters")
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if not isinstance(g, torch.Tensor):
+                raise TypeError(f"Muon: gradient {i} is no tensor: {type(g).__name__}")
+            # the entry below sees matrices of as many elements
+            if g.shape != p.shape and tuple(g.shape) != (p.shape[0], math.prod(p.shape[1:])):
+                raise VoltaHipError(_lib.VH_ERR_BAD_SHAPE, f"Muon: gradient {i} is {tuple(g.shape)}, its parameter {tuple(p.shape)}")
+            if g.device != p.device or not p.is_cuda:
+                raise VoltaHipError(_lib.VH_ERR_NO_DEVICE, f"Muon: the tensors must be on one device, gradient {i} is on {g.device}, "
+                                                           f"its parameter on {p.device}")
+            _same_dtype(p, g)
+            if not (g.is_contiguous() and p.is_contiguous()):
+                raise ValueError(f"Muon: parameter {i} and its gradient must be contiguous")
         for p, g, m in zip(self.params, grads, self.momentum):
             rows = p.shape[0]
             _on_device(ops.gpu_muon_step(p.view(rows, -1), g.view(rows, -1), m.view(rows, -1), self.lr, self.beta,
