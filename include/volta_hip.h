@@ -472,7 +472,9 @@ int vh_orthogonalize(int dtype, const void* grad, void* out, int64_t batch, int6
 /* One optimiser step on a batch of matrices, in place:
  *   momentum <- beta momentum + grad;  u = nesterov ? grad + beta momentum : momentum
  *   params <- (1 - lr weight_decay) params - lr sqrt(max(1, rows / cols)) orthogonalize(u)
- * params and grads of `dtype`, momentum fp32. */
+ * params and grads of `dtype`, momentum fp32.  rows / cols is outputs / inputs of a weight that lies
+ * [out][in]; one that lies [in][out], as Linear's, has its factor with lr sqrt(cols / rows) for lr and
+ * weight_decay sqrt(rows / cols) for weight_decay. */
 int vh_muon_step(int dtype, void* params, const void* grads, float* momentum, int64_t batch, int64_t rows, int64_t cols,
                  float lr, float beta, float weight_decay, int nesterov, int steps, float eps, void* stream);
 

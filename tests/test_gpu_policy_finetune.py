@@ -99,3 +99,58 @@ def test_muon_refuses_before_it_updates():
     good[1] = good[1].view(24, 54)  # a kernel's matrix
     opt.step(good)
     assert not any(torch.equal(a, b) for a, b in zip(params + opt.momentum, before))
+
+
+def _steps_of(u):
+    x = u.mT.contiguous() if u.shape[-2] > u.shape[-1] else u
+    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + 1e-7)
+    for _ in range(5):
+        gram = x @ x.mT.contiguous()
+        x = 3.4445 * x + (-4.7750 * gram + 2.0315 * (gram @ gram)) @ x
+    return x.mT.contiguous() if u.shape[-2] > u.shape[-1] else x
+
+
+@pytest.mark.parametrize("inputs,outputs", [(96, 400), (400, 96), (784, 512), (64, 64), (10, 300)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_muon_steps_go_by_inputs_and_outputs(inputs, outputs, dtype):
+    """A layer's update is scaled by sqrt(max(1, outputs / inputs)) however its weight lies: a Linear's [in, out], a
+    Conv2d's [out, in, k, k], a ConvTranspose2d's [in, out, k, k].  Tolerances: the parameters' own rounding, and
+    the update's error, 1e-4 of it in fp32 and 4e-3 in bf16."""
+    lr, wd, beta = 0.05, 0.1, 0.9
+    gen = torch.Generator().manual_seed(7)
+    c_in, c_out = max(1, inputs // 8), max(1, outputs // 8)
+    layers = ((nn.Linear(inputs, outputs, device=DEV, dtype=dtype, generator=gen), None, inputs, outputs),
+              (nn.Conv2d(c_in, c_out, 3, device=DEV, dtype=dtype, generator=gen), None, c_in * 9, c_out),
+              (nn.ConvTranspose2d(c_in, c_out, 3, device=DEV, dtype=dtype, generator=gen), True, c_in, c_out * 9))
+    for layer, in_first, ins, outs in layers:
+        w = layer.weight
+        grad = torch.randn(w.shape, generator=torch.Generator(device=DEV).manual_seed(8), device=DEV).to(dtype)
+        opt = nn.Muon([w], lr=lr, beta=beta, weight_decay=wd, in_first=in_first)
+        for _ in range(2):
+            old, m64 = w.double(), beta * opt.momentum[0].double() + grad.double()
+            rows = w.shape[0]
+            u = (grad.double() + beta * m64).view(rows, -1)
+            update = (lr * max(1.0, outs / ins) ** 0.5 * _steps_of(u)).view(w.shape)
+            opt.step([grad])
+            want = old * (1 - lr * wd) - update
+            off = float(torch.linalg.vector_norm(w.double() - want))
+            own, step = float(torch.linalg.vector_norm(want)), float(torch.linalg.vector_norm(update))
+            assert off <= (2.0 ** -8 * own + 4e-3 * step if dtype == torch.bfloat16 else 2.0 ** -23 * own + 1e-4 * step), \
+                (type(layer).__name__, off, own, step)
+
+
+def test_muon_takes_an_orientation_for_each_parameter():
+    g = torch.Generator(device=DEV).manual_seed(9)
+    w = torch.randn((20, 80), generator=g, device=DEV)
+    dw = torch.randn((20, 80), generator=g, device=DEV)
+    apart = []
+    for in_first in (True, False):
+        p = w.clone()
+        nn.Muon([p], lr=0.1, in_first=in_first).step([dw])
+        apart.append(p)
+    assert torch.allclose((w - apart[0]) / 2, w - apart[1], rtol=0, atol=1e-6)  # sqrt(80 / 20) = 2
+    a, b = w.clone(), w.clone()
+    nn.Muon([a, b], lr=0.1, in_first=[True, False]).step([dw, dw])
+    assert torch.equal(a, apart[0]) and torch.equal(b, apart[1])
+    with pytest.raises(ValueError):
+        nn.Muon([a, b], in_first=[True])

@@ -357,14 +357,23 @@ class PreferenceLoss:
 class Muon:
     """The orthogonalised-momentum optimiser (gpu_muon_step) over weight matrices: Linear's [in, out], a
     convolution's [out, in, k, k] as [out, in * k * k].  Holds an fp32 momentum for each; step(grads) updates the
-    parameters in place."""
+    parameters in place.
+
+    An update is scaled by sqrt(max(1, outputs / inputs)).  Which of a matrix's sides is the inputs' is ``in_first``: a
+    bool, or one for each parameter; None: the first of two dimensions (Linear), the last ones of more (Conv2d).  A
+    ConvTranspose2d's [in, out, k, k] takes True."""
 
     def __init__(self, params, lr: float = 0.02, beta: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True,
-                 steps: int = 5, eps: float = 1e-7):
+                 steps: int = 5, eps: float = 1e-7, in_first=None):
         self.params = list(params)
         for p in self.params:
             if p.dim() < 2:
                 raise VoltaHipError(_lib.VH_ERR_BAD_SHAPE, f"Muon: a matrix or a kernel, got {tuple(p.shape)}")
+        if in_first is None:
+            in_first = [p.dim() == 2 for p in self.params]
+        self.in_first = [in_first] * len(self.params) if isinstance(in_first, bool) else list(in_first)
+        if len(self.in_first) != len(self.params):
+            raise ValueError(f"Muon: {len(self.in_first)} orientations for {len(self.params)} parameters")
         self.momentum = [torch.zeros(p.shape, dtype=torch.float32, device=p.device) for p in self.params]
         self.lr, self.beta, self.weight_decay = lr, beta, weight_decay
         self.nesterov, self.steps, self.eps = nesterov, steps, eps
@@ -387,10 +396,10 @@ class Muon:
             _same_dtype(p, g)
             if not (g.is_contiguous() and p.is_contiguous()):
                 raise ValueError(f"Muon: parameter {i} and its gradient must be contiguous")
-        for p, g, m in zip(self.params, grads, self.momentum):
+        for p, g, m, in_first in zip(self.params, grads, self.momentum, self.in_first):
             rows = p.shape[0]
             _on_device(ops.gpu_muon_step(p.view(rows, -1), g.view(rows, -1), m.view(rows, -1), self.lr, self.beta,
-                                         self.weight_decay, self.nesterov, self.steps, self.eps), "Muon")
+                                         self.weight_decay, self.nesterov, self.steps, self.eps, in_first), "Muon")
 
 
 class ConvChain:

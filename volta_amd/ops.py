@@ -10,6 +10,7 @@ raise (the reference panics there).  Outputs are allocated by the callee, as
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -511,14 +512,21 @@ def gpu_orthogonalize(grad: torch.Tensor, steps: int = 5, eps: float = 1e-7, out
 
 @_optional
 def gpu_muon_step(params: torch.Tensor, grads: torch.Tensor, momentum: torch.Tensor, lr: float, beta: float = 0.95,
-                  weight_decay: float = 0.0, nesterov: bool = True, steps: int = 5, eps: float = 1e-7):
+                  weight_decay: float = 0.0, nesterov: bool = True, steps: int = 5, eps: float = 1e-7,
+                  in_first: bool = False):
     """One step of the orthogonalised-momentum optimiser on a matrix, or on each of a batch; params and momentum
     (float32) are updated in place:
 
     momentum = beta momentum + grads; u = grads + beta momentum (nesterov) or momentum;
-    params = (1 - lr weight_decay) params - lr sqrt(max(1, rows / cols)) orthogonalize(u)."""
+    params = (1 - lr weight_decay) params - lr sqrt(max(1, outputs / inputs)) orthogonalize(u),
+
+    with rows for outputs and cols for inputs, or, ``in_first``, as Linear's weights lie, the other way round."""
     what = "gpu_muon_step"
     batch, rows, cols = _matrices(params, what)
+    if in_first and rows != cols and rows and cols:
+        # the entry's factor is that of [out, in]: what it is to be over what it will be, in lr, and out of the decay
+        ratio = math.sqrt(cols / rows)
+        lr, weight_decay = lr * ratio, weight_decay / ratio
     dt = _same_dtype(params, grads)
     if momentum.dtype != torch.float32:
         raise TypeError(f"{what}: momentum is float32")
