@@ -464,7 +464,8 @@ int vh_residual_norm_backward(int dtype, const void* grad_y, const void* grad_n,
 /* ---- Orthogonalised updates (the Muon optimiser of src/nn/optim/, on the device) ----
  * Newton-Schulz: with X = G / (|G|_F + eps) (a matrix taller than wide transposed),
  *   A = X X^T,  X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X    `steps` times (1 .. 64; 5 is usual)
- * takes G's singular values to about 1 (0.7 .. 1.2) and keeps its singular vectors.  `grad` and
+ * takes G's singular values to about 1 (0.7 .. 1.2) and keeps its singular vectors; zeros stay zeros, with
+ * eps = 0 too.  `grad` and
  * `out` are [batch][rows][cols], batch under 2^22; out may be grad.  VH_F32 is computed to fp32's accuracy; VH_BF16
  * with fp16 products and fp32 sums and diagonals, its error below the output's rounding. */
 int vh_orthogonalize(int dtype, const void* grad, void* out, int64_t batch, int64_t rows, int64_t cols, int steps,

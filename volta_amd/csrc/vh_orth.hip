@@ -425,6 +425,20 @@ __device__ __forceinline__ void update8(const LoadArgs& p, size_t i, long n, flo
   }
 }
 
+// What takes a matrix of Frobenius norm sqrt(s) to planes of norm kSX: factor times two to the power k.  As
+// one fp32 it would be infinite from entries of 1e-37 on and lose bits for norms past 1e41; in two,
+// an entry is scaled by the power, which is exact, then rounded once.  Where there is nothing to divide by,
+// zeros stay zeros.
+struct Scale {
+  float factor;
+  int k;
+  __device__ __forceinline__ float operator()(float v) const { return __builtin_amdgcn_ldexpf(v, k) * factor; }
+};
+__device__ __forceinline__ Scale scale_of(double s, float eps) {
+  const double norm = sqrt(s) + (double)eps, d = norm == 0.0 ? 0.0 : (double)kSX / norm;
+  return {(float)__builtin_amdgcn_frexp_mant(d), __builtin_amdgcn_frexp_exp(d)};
+}
+
 // mom = beta mom + v; v = what is orthogonalised
 __device__ __forceinline__ void new_momentum8(const LoadArgs& p, size_t i, long n, float (&v)[8]) {
   float m[8];
@@ -496,12 +510,12 @@ __global__ __launch_bounds__(256) void orth_load_kernel(LoadArgs p) {
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  const float f = (float)(kSX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + (double)p.eps));
+  const Scale f = scale_of((red[0] + red[1]) + (red[2] + red[3]), p.eps);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int r = lr + 32 * k;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[k][e] = (TALL ? tile[lc + e][r] : v[k][e]) * f;
+    for (int e = 0; e < 8; ++e) v[k][e] = f(TALL ? tile[lc + e][r] : v[k][e]);
     const size_t o = blockIdx.z * p.zo + (size_t)(i0 + r) * p.ld + j0 + lc;
     store8(p.out[0] + o, p.out[1] + o, v[k]);
   }
@@ -688,7 +702,7 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32) * G) void orth_small_ker
   __syncthreads();
   s = 0;
   for (int w = 0; w < WAVES; ++w) s += red[w];
-  const float f = (float)(kSX / (sqrt(s) + (double)l.eps));
+  const Scale f = scale_of(s, l.eps);
   const int cols = p.tall ? p.m : p.n;  // of the matrix as it lies
   for (long i = tid * 8; i < l.z; i += THREADS * 8) {
     float v[8];
@@ -697,7 +711,7 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32) * G) void orth_small_ker
     if (!p.tall && cols % 8 == 0) {
       const int at = small_at<MP>(r, c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= f;
+      for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
       store8(reinterpret_cast<_Float16*>(X[0] + at), reinterpret_cast<_Float16*>(X[1] + at), v);
     } else {
 #pragma unroll
@@ -705,7 +719,7 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32) * G) void orth_small_ker
         if (i + e < l.z) {
           const int at = p.tall ? small_at<MP>(c, r) : small_at<MP>(r, c);
           _Float16 h, q;
-          split(v[e] * f, h, q);
+          split(f(v[e]), h, q);
           *reinterpret_cast<_Float16*>(X[0] + at) = h;
           *reinterpret_cast<_Float16*>(X[1] + at) = q;
         }
@@ -844,7 +858,8 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32) * G) void orth_slice_ker
   const int ri = wi * 32 + row_l, aj = wj * 32;
   auto col_of = [&](int c0, int q) { return c0 + 8 * q + 4 * half_l; };
   f16x8 a[2], b[2];
-  float f = 0.f, di = 0.f;
+  Scale f{};
+  float di = 0.f;
 
   if constexpr (FIRST) {
     double s = 0;
@@ -855,7 +870,7 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32) * G) void orth_slice_ker
     __syncthreads();
     s = 0;
     for (int w = 0; w < WAVES; ++w) s += red[w];
-    f = (float)(kSX / (sqrt(s) + (double)l.eps));
+    f = scale_of(s, l.eps);
   } else {
     // A: the slices' parts added in order
     const float* part = p.part_in + (size_t)z * p.slices * MP * MP;
@@ -909,14 +924,14 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32) * G) void orth_slice_ker
         if (!p.tall) {
           const int at = small_at<MP>(r, e0);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= f;
+          for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
           store8(reinterpret_cast<_Float16*>(X[0] + at), reinterpret_cast<_Float16*>(X[1] + at), v);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int at = small_at<MP>(r + e, o);
             _Float16 h, q;
-            split(v[e] * f, h, q);
+            split(f(v[e]), h, q);
             *reinterpret_cast<_Float16*>(X[0] + at) = h;
             *reinterpret_cast<_Float16*>(X[1] + at) = q;
           }
