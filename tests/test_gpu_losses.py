@@ -372,3 +372,20 @@ def test_policy_loss_rows_are_the_same_among_many(vocab, dtype):
     assert torch.equal(logp[:1024], ops.gpu_policy_loss(x[:1024], tokens[:1024], old[:1024], adv[:1024])[1])
     a, b = (ops.gpu_policy_loss(x[:n], tokens[:n], old[:n], adv[:n], mask=torch.arange(n, device=DEV) < 9)[2] for n in (1030, 1024))
     assert torch.equal(a[:1024], b) and not b[9:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,temperature", [(9, 203, 1.0), (300, 2067, 0.9), (40, 5003, 1.0), (300, 32003, 0.9), (20, 65533, 1.3), (3, 140001, 0.9)])
+def test_policy_gradient_is_one_function_of_the_logit(rows, vocab, temperature, dtype):
+    """Entries of a row with the same logit have the same gradient bit for bit, whichever thread writes them (the last
+    unit of an odd row is written by two), and every call gives the same."""
+    x, tokens, old, adv, ref = make(rows, vocab, dtype, seed=21)
+    same = torch.arange(vocab, device=DEV) % 5 == 0
+    x[:, same] = x[:, :1]
+    tokens = (tokens // 5 * 5 + 1) % (vocab // 5 * 5)  # none of them
+    old = ops.gpu_token_logprobs(x, tokens, temperature) + 0.1
+    call = lambda: ops.gpu_policy_loss(x, tokens, old, adv, old, None, 0.2, 0.2, 0.1, temperature)  # noqa: E731
+    first = call()
+    assert torch.equal(first[2][:, same], first[2][:, :1].expand(-1, int(same.sum())))
+    for _ in range(10):
+        assert all(torch.equal(a, b) for a, b in zip(call(), first))

@@ -60,8 +60,10 @@ __device__ __forceinline__ void add_unit(MaxSum& a, const Unit<T>& u, float inv_
   a = {m, s};
 }
 
-// Of the whole row, in every one of its THREADS threads; each wave's values are joined in
-// the same order.
+// Of the whole row, in every one of its THREADS threads the same: the two sides of a join are
+// rounded differently (the first product within a multiply-add), so the lanes of a wave end with
+// sums that differ in their last bits.  The first lane's is taken, which in each wave
+// is joined in the same order.
 template <int THREADS>
 __device__ __forceinline__ MaxSum block_join(MaxSum a, MaxSum* red) {
 #pragma unroll
@@ -80,7 +82,8 @@ __device__ __forceinline__ MaxSum block_join(MaxSum a, MaxSum* red) {
       a = join(a, b);
     }
   }
-  return a;
+  auto first = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); };
+  return {first(a.m), first(a.s)};
 }
 
 __device__ __forceinline__ bool tok_ok(long tok, int V) {
