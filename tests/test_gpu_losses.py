@@ -389,3 +389,21 @@ def test_policy_gradient_is_one_function_of_the_logit(rows, vocab, temperature, 
     assert torch.equal(first[2][:, same], first[2][:, :1].expand(-1, int(same.sum())))
     for _ in range(10):
         assert all(torch.equal(a, b) for a, b in zip(call(), first))
+
+
+@pytest.mark.parametrize("smooth", [0.0, 1.0, 0.3])
+@pytest.mark.parametrize("margin", [-80.0, -45.0, -30.0, -3.0, 3.0, 30.0, 36.0, 45.0, 80.0])
+def test_preference_gradient_of_a_decided_pair(margin, smooth):
+    """The slope e sigmoid(z) - (1 - e) sigmoid(-z) to fp32's accuracy where sigmoid(z) is all but 0 or 1: a
+    log-probability off by 8e-6 changes it by as much of itself, the row's own terms add 2e-5."""
+    x, tokens, *_ = make(3, 70, torch.float32, seed=11)
+    offsets = torch.tensor([0, 1, 3], device=DEV)
+    _, logp = ref_logp64(x, tokens)
+    refs = torch.stack((logp[0] - margin, logp[1:].sum())).float()
+    _, _, grad = ops.gpu_preference_loss(x, tokens, offsets, refs, None, 1.0, smooth)
+    z = (logp[0] - refs[0].double()) - (logp[1:].sum() - refs[1].double())
+    c = smooth * torch.sigmoid(z) - (1 - smooth) * torch.sigmoid(-z)
+    onehot = torch.zeros_like(x, dtype=torch.float64).scatter_(1, tokens[:, None], 1.0)
+    want = torch.stack((c, -c, -c))[:, None] * (onehot - x.double().softmax(1))
+    off = (grad.double() - want).abs().amax(1)
+    assert bool((off <= 1e-4 * want.abs().amax(1)).all()), (off / want.abs().amax(1)).tolist()
