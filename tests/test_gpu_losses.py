@@ -407,3 +407,21 @@ def test_preference_gradient_of_a_decided_pair(margin, smooth):
     want = torch.stack((c, -c, -c))[:, None] * (onehot - x.double().softmax(1))
     off = (grad.double() - want).abs().amax(1)
     assert bool((off <= 1e-4 * want.abs().amax(1)).all()), (off / want.abs().amax(1)).tolist()
+
+
+def test_preference_loss_of_impossible_answers():
+    """A sequence that holds a token of probability 0 has lost (a loss of 0 if it is the rejected one, of infinity if
+    the preferred one); labels that name one side only do not look at the other's logarithm."""
+    x, tokens, *_ = make(4, 40, torch.float32, seed=12)
+    tokens[1], x[1, 3] = 3, -INF
+    offsets = torch.tensor([0, 2, 4], device=DEV)  # sequence 0 has the row, sequence 1 not
+    swap = torch.tensor([2, 3, 0, 1], device=DEV)
+    refs = torch.tensor([-5.0, -6.0], device=DEV)
+    for smooth, lost in ((0.0, True), (1.0, False)):
+        loss, seq, _ = ops.gpu_preference_loss(x, tokens, offsets, refs, None, 0.5, smooth)
+        assert float(seq[0]) == -INF and float(loss) == (INF if lost else 0.0)
+        loss, seq, grad = ops.gpu_preference_loss(x[swap], tokens[swap], offsets, refs, None, 0.5, smooth)
+        assert float(seq[1]) == -INF and float(loss) == (0.0 if lost else INF)
+        assert torch.isfinite(grad).all() and (not lost or not grad.any())
+    loss, _, _ = ops.gpu_preference_loss(x, tokens, offsets, refs, None, 0.5, 0.3)
+    assert float(loss) == INF

@@ -414,7 +414,8 @@ __global__ __launch_bounds__(128) void pair_kernel(PairArgs p) {
   __syncthreads();
   if (threadIdx.x) return;
   const double z = (double)p.beta * (sum[0] - sum[1]), e = p.smooth;
-  p.term[blockIdx.x] = (1 - e) * log1p_exp(-z) + e * log1p_exp(z);
+  // an infinite margin (a token of probability 0): a label's share of 0 is none, not 0 infinity
+  p.term[blockIdx.x] = (e < 1 ? (1 - e) * log1p_exp(-z) : 0.0) + (e > 0 ? e * log1p_exp(z) : 0.0);
   // e sigmoid(z) - (1 - e) sigmoid(-z): a difference of sigmoid(z) and 1 - e loses what is left of a
   // decided pair's slope (1e-3 of it at z = 30, all of it at 37)
   const double d = p.beta / p.pairs * (e / (1.0 + exp(-z)) - (1 - e) / (1.0 + exp(z)));
