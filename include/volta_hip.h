@@ -417,8 +417,8 @@ int vh_token_logprobs(int dtype, const void* logits, int64_t logits_stride, cons
 /* The clipped policy loss: with r = exp(logp - old_logp), A the row's advantage and
  * d = ref_logp - logp,
  *   loss = 1/M sum_rows [ -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1) ]
- * over the M rows that the mask keeps (M at least 1).  `loss` is one fp32, `logp` [rows]
- * receives the rows' log-probabilities.  ref_logp may be NULL when kl_coef is 0. */
+ * over the M rows that the mask keeps (M at least 1).  In the gradient r, e^d and a row's coefficient are at
+ * most fp32's largest value.  `loss` is one fp32, `logp` [rows] receives the rows' log-probabilities.  ref_logp may be NULL when kl_coef is 0. */
 int vh_policy_loss(int dtype, const void* logits, int64_t logits_stride, const void* tokens, const float* old_logp,
                    const float* advantages, const float* ref_logp, const void* mask, float* loss, float* logp,
                    void* grad_logits, int64_t grad_stride, int64_t rows, int64_t vocab, float clip_low,

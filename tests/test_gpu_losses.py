@@ -425,3 +425,22 @@ def test_preference_loss_of_impossible_answers():
         assert torch.isfinite(grad).all() and (not lost or not grad.any())
     loss, _, _ = ops.gpu_preference_loss(x, tokens, offsets, refs, None, 0.5, 0.3)
     assert float(loss) == INF
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_policy_loss_of_far_ratios(dtype):
+    """Ratios and KL terms whose exponential passes fp32: a row without an advantage has no gradient by its ratio, one
+    past the clip none either, and nothing turns into NaN where entries have probability 0."""
+    x, tokens, old, adv, ref = make(6, 300, dtype, seed=13)
+    tokens %= 200
+    x[:, 250:] = -INF
+    logp = ops.gpu_token_logprobs(x, tokens)
+    old = logp + torch.tensor([-100.0, -300.0, -0.1, -100.0, -95.0, 0.2], device=DEV)
+    adv = torch.tensor([0.0, 0.0, 0.5, 2.0, -1.0, -0.3], device=DEV)
+    _, grad = check_policy(x[:4], tokens[:4], old[:4], adv[:4], None, None, kl=0.0)
+    assert not grad[0].any() and not grad[1].any() and grad[2].any() and not grad[3].any()
+    _, _, grad = ops.gpu_policy_loss(x, tokens, old, adv)
+    assert torch.isfinite(grad).all() and not grad[:, 250:].any() and grad[4].abs().max() > 1e37
+    ref = logp + torch.tensor([0.1, 0.1, 0.1, 100.0, 0.1, 0.1], device=DEV)
+    _, _, grad = ops.gpu_policy_loss(x, tokens, old, adv, ref, None, 0.2, 0.2, 0.05)
+    assert torch.isfinite(grad).all() and not grad[:, 250:].any()

@@ -119,6 +119,13 @@ __device__ __forceinline__ void grad_unit(Unit<T>& u, int at, float inv_t, float
 }
 
 // ---------------------------------------------------------------- the policy loss
+// Ratios and KL terms past fp32 count as its largest value in the gradient, as does the
+// row's coefficient: infinite, they would turn an advantage of 0 and every entry of
+// probability 0 into NaN.  A NaN stays one.
+constexpr float kMost = 3.402823466e38f;
+__device__ __forceinline__ float finite(float v) { return fabsf(v) > kMost ? copysignf(kMost, v) : v; }
+__device__ __forceinline__ float exp_finite(float v) { return finite(expf(v)); }
+
 struct PolicyArgs {
   const void* logits;
   long ld;
@@ -237,17 +244,17 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void policy_kernel(P
   }
   a = block_join<THREADS>(a, red);
   const double logp = logp_of(zt, a);
-  const float ratio = expf((float)(logp - (double)old));
+  const float ratio = exp_finite((float)(logp - (double)old));
   const float plain = ratio * adv, clipped = fminf(fmaxf(ratio, 1.f - p.lo), 1.f + p.hi) * adv;
   float d = plain <= clipped ? -plain : 0.f;  // the loss's slope in logp
   if (isnan(plain)) d = plain;  // min and max leave a NaN out
-  if (p.ref_logp && p.kl != 0.f) d += p.kl * (1.f - expf((float)((double)p.ref_logp[row] - logp)));
+  if (p.ref_logp && p.kl != 0.f) d += p.kl * (1.f - exp_finite((float)((double)p.ref_logp[row] - logp)));
   // The row's loss behind its gradient, by one wave: in double, for the loss is a small
   // difference of terms where advantages cancel, and of a few rows the terms' last bits in
   // fp32 were 4e-6 of it.
   auto loss_term = [&] {
     if (tid) return;
-    const double r = exp(logp - (double)old), full = r * adv;
+    const double r = exp(logp - (double)old), full = adv == 0.f && r > 0.0 ? 0.0 : r * adv;
     double term = -fmin(full, fmin(fmax(r, 1.0 - (double)p.lo), 1.0 + (double)p.hi) * adv);
     if (isnan(full)) term = full;
     if (p.ref_logp && p.kl != 0.f) {
@@ -258,7 +265,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void policy_kernel(P
     p.term[row] = term;
   };
   if (!g) return loss_term();
-  const float c = d * p.inv_t * p.grad_scale / count, cs = -c / a.s, m = finite_or_0(a.m);
+  const float c = finite(d * p.inv_t * p.grad_scale / count), cs = -c / a.s, m = finite_or_0(a.m);
 #pragma unroll
   for (int i = 0; i < NU; ++i) {
     if ((i + 1) * THREADS < units) {
