@@ -408,7 +408,7 @@ int vh_optimizer_step(int op, float lr, float beta1, float beta2, float t, float
  * 0 is not read, whatever its logits and token hold; it adds nothing to the loss, its logp
  * is 0 and its gradient zeros.  `grad_logits` (stride `grad_stride`, the logits' dtype)
  * receives grad_scale * dLoss/dlogits; NULL skips it; it may be the logits themselves
- * (same pointer and stride), or not overlap them.  Sums run in a fixed order.  A launch
+ * (same pointer and stride), or share no element with them (another column range of their table at most).  Sums run in a fixed order.  A launch
  * has fewer than 2^32 threads: rows of up to 2 KiB may number 2^26 less 16, of up to 32 KiB
  * 2^24 less 16, longer ones 2^22 less 16, pairs 2^25 less 16. */
 /* logp [rows] of each row's token: what old_logp and ref_logp below are made with. */

@@ -444,3 +444,28 @@ def test_policy_loss_of_far_ratios(dtype):
     ref = logp + torch.tensor([0.1, 0.1, 0.1, 100.0, 0.1, 0.1], device=DEV)
     _, _, grad = ops.gpu_policy_loss(x, tokens, old, adv, ref, None, 0.2, 0.2, 0.05)
     assert torch.isfinite(grad).all() and not grad[:, 250:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [7, 333, 2051])
+def test_logits_and_gradient_beside_each_other(vocab, dtype):
+    """Two column ranges of one table share no element; ranges that do are refused, around a row's end too."""
+    rows = 5
+    x, tokens, old, adv, ref = make(rows, vocab, dtype, seed=14)
+    offsets, refs = torch.tensor([0, 2, 5], device=DEV), torch.tensor([-3.0, -4.0], device=DEV)
+    want = ops.gpu_policy_loss(x, tokens, old, adv, ref), ops.gpu_preference_loss(x, tokens, offsets, refs)
+    for first, second, width in ((0, vocab, 2 * vocab), (vocab + 3, 1, 2 * vocab + 5), (2, vocab + 9, 2 * vocab + 11)):
+        table = torch.full((rows, width), 5.0, dtype=dtype, device=DEV)
+        a, b = table[:, first:first + vocab], table[:, second:second + vocab]
+        a.copy_(x)
+        assert all(torch.equal(p, q) for p, q in zip(ops.gpu_policy_loss(a, tokens, old, adv, ref, out=b), want[0]))
+        assert all(torch.equal(p, q) for p, q in zip(ops.gpu_preference_loss(a, tokens, offsets, refs, out=b), want[1]))
+        assert torch.equal(a, x)
+        table[:, first:first + vocab], table[:, second:second + vocab] = 5.0, 5.0
+        assert bool((table == 5).all())
+    flat = torch.zeros(rows * 3 * vocab, dtype=dtype, device=DEV)
+    for stride, at in ((2 * vocab, vocab - 1), (2 * vocab, vocab + 1), (2 * vocab - 1, vocab), (2 * vocab, 2 * vocab - 1)):
+        a, b = (flat.as_strided((rows, vocab), (stride, 1), o) for o in (0, at))
+        for p, q in ((a, b), (b, a)):
+            with pytest.raises(volta_amd.VoltaHipError):
+                ops.gpu_policy_loss(p, tokens, old, adv, out=q)

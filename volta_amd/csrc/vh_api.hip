@@ -1884,7 +1884,8 @@ static int check_logits(int dtype, const void* logits, int64_t stride, int64_t r
   if (reinterpret_cast<uintptr_t>(logits) % elem_size(dtype)) return set_error(VH_ERR_BAD_ARG, "logits off their element's alignment");
   return VH_OK;
 }
-// grad may be the logits (the same rows) or apart from them
+// grad may be the logits (the same rows) or apart from them: outside all of them, or another range of columns
+// of the same table
 static int check_logits_grad(int dtype, const void* logits, int64_t stride, const void* grad, int64_t grad_stride,
                              int64_t rows, int64_t vocab) {
   if (!grad) return VH_OK;
@@ -1897,8 +1898,12 @@ static int check_logits_grad(int dtype, const void* logits, int64_t stride, cons
   if (rows == 0) return VH_OK;
   const uintptr_t es = elem_size(dtype), a = reinterpret_cast<uintptr_t>(logits), b = reinterpret_cast<uintptr_t>(grad);
   const uintptr_t an = ((uintptr_t)(rows - 1) * stride + vocab) * es, bn = ((uintptr_t)(rows - 1) * grad_stride + vocab) * es;
-  if (a < b + bn && b < a + an) return set_error(VH_ERR_BAD_ARG, "the gradient overlaps the logits");
-  return VH_OK;
+  if (a >= b + bn || b >= a + an) return VH_OK;
+  if (stride == grad_stride) {
+    const uintptr_t row = (uintptr_t)stride * es, off = a < b ? (b - a) % row : (row - (a - b) % row) % row, used = (uintptr_t)vocab * es;
+    if (off >= used && off + used <= row) return VH_OK;
+  }
+  return set_error(VH_ERR_BAD_ARG, "the gradient overlaps the logits");
 }
 
 int vh_token_logprobs(int dtype, const void* logits, int64_t logits_stride, const void* tokens, float* logp,
