@@ -447,14 +447,15 @@ int vh_preference_loss(int dtype, const void* logits, int64_t logits_stride, con
  * the rows / gate_rows rows from g * rows / gate_rows on (1: one learned vector, the number
  * of sequences: one each, rows: one for each row).  rstd [2][rows] receives 1 / rms of
  * block (1 without post_weight) and of y (1 without next_weight), for the backward.
- * n is made from y before y's rounding.  y may be x, n may be block. */
+ * n is made from y before y's rounding.  y may be x, n may be block; outputs that overlap an input in part, or
+ * each other, are refused (VH_ERR_BAD_ARG). */
 int vh_residual_norm(int dtype, const void* x, const void* block, const void* gate, const void* post_weight,
                      const void* next_weight, void* y, void* n, float* rstd, int64_t rows, int64_t width,
                      int64_t gate_rows, float scale, float eps, void* stream);
 /* Its backward, from grad_y (NULL: nothing but n uses y) and grad_n (with next_weight):
  * grad_x and grad_block, and the gradient of every gate and weight that is given, summed
  * over the rows that share it in a fixed order (0 where there are no rows).  x, block and rstd are the forward's.
- * grad_x may be grad_y, grad_block may be grad_n or block. */
+ * grad_x may be grad_y, grad_block may be grad_n or block; overlaps are refused as the forward's. */
 int vh_residual_norm_backward(int dtype, const void* grad_y, const void* grad_n, const void* x, const void* block,
                               const float* rstd, const void* gate, const void* post_weight, const void* next_weight,
                               void* grad_x, void* grad_block, void* grad_gate, void* grad_post_weight,

@@ -283,3 +283,33 @@ def test_no_rows_leave_the_gate_no_gradient(dtype):
     del junk  # the next allocation of this size
     dgate = ops.gpu_residual_norm_backward(t["dy"], t["dn"], t["x"], t["b"], rstd, t["gate"], t["wp"], t["wn"])[2]
     assert dgate.shape == (1, width) and not dgate.any()
+
+
+def test_refuses_outputs_that_overlap_in_part():
+    """By the addresses alone.  An output may lie on an input of its size as a whole, or apart from all of them."""
+    lib, s = _lib.lib(), ops.stream_ptr(torch.device(DEV))
+    rows, width = 6, 40
+    n = rows * width * 4
+    buf = torch.ones(40 * n, dtype=torch.uint8, device=DEV)
+    at = lambda i, off=0: buf.data_ptr() + i * 2 * n + off  # noqa: E731
+    x, b, gate, wp, wn, y, out, rstd, dy, dn, dx, db, dgate, dwp, dwn = (at(i) for i in range(15))
+
+    def forward(y=y, out=out, rstd=rstd):
+        return lib.vh_residual_norm(0, x, b, gate, wp, wn, y, out, rstd, rows, width, 2, 1.0, 1e-6, s)
+
+    def backward(dx=dx, db=db, dgate=dgate, dwp=dwp, dwn=dwn):
+        return lib.vh_residual_norm_backward(0, dy, dn, x, b, rstd, gate, wp, wn, dx, db, dgate, dwp, dwn, rows, width, 2, 1.0, s)
+
+    row = width * 4
+    for call, wrong in ((forward, dict(y=x + row)), (forward, dict(y=b - row)), (forward, dict(out=b + 4)), (forward, dict(out=x + n - 4)),
+                        (forward, dict(y=gate)), (forward, dict(out=wn)), (forward, dict(out=y)), (forward, dict(out=y + row)),
+                        (forward, dict(rstd=x)), (forward, dict(rstd=y + 8)), (forward, dict(rstd=wp)),
+                        (backward, dict(dx=dy + row)), (backward, dict(db=dn - 4)), (backward, dict(db=b + row)), (backward, dict(dx=x + 4)),
+                        (backward, dict(dx=rstd)), (backward, dict(dgate=gate + row)), (backward, dict(dgate=dn)),
+                        (backward, dict(dwp=wp + 4)), (backward, dict(dwn=dwp)), (backward, dict(db=dx)), (backward, dict(dwp=dgate + row)),
+                        (backward, dict(dwn=rstd + 8))):
+        assert call(**wrong) == _lib.VH_ERR_BAD_ARG, wrong
+    for call, right in ((forward, {}), (forward, dict(y=x, out=b)), (forward, dict(y=x + n, out=b + n)), (backward, {}),
+                        (backward, dict(dx=dy, db=dn)), (backward, dict(dx=dy, db=b)), (backward, dict(dwp=wp, dwn=wn, dgate=gate))):
+        assert call(**right) == _lib.VH_OK, right
+    torch.cuda.synchronize()

@@ -1955,6 +1955,27 @@ int vh_preference_loss(int dtype, const void* logits, int64_t logits_stride, con
   return VH_DISPATCH(dtype, run_preference_loss, q, (float*)ws, st);
 }
 
+// Outputs share no memory with one another, nor with an input but as a whole (its place and size: a thread
+// writes there what it alone has read), and that not where one of the two is `alone`.
+struct Range {
+  const void* p;
+  size_t bytes;
+  bool alone = false;
+};
+static int check_apart(std::initializer_list<Range> outs, std::initializer_list<Range> ins) {
+  auto overlap = [](const Range& a, const Range& b) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a.p), q = reinterpret_cast<uintptr_t>(b.p);
+    return p && q && p < q + b.bytes && q < p + a.bytes;
+  };
+  for (const Range* o = outs.begin(); o != outs.end(); ++o) {
+    for (const Range* other = o + 1; other != outs.end(); ++other)
+      if (overlap(*o, *other)) return set_error(VH_ERR_BAD_ARG, "outputs overlap");
+    for (const Range& i : ins)
+      if (overlap(*o, i) && (o->alone || i.alone || o->p != i.p || o->bytes != i.bytes)) return set_error(VH_ERR_BAD_ARG, "an output overlaps an input in part");
+  }
+  return VH_OK;
+}
+
 // ------------------------------------------------------------------ gated residual norms
 static int check_norm(int dtype, const void* gate, int64_t rows, int64_t width, int64_t gate_rows) {
   VH_TRY(check_dtype(dtype));
@@ -1979,6 +2000,9 @@ int vh_residual_norm(int dtype, const void* x, const void* block, const void* ga
   if (!(eps >= 0.f)) return set_error(VH_ERR_BAD_ARG, "eps must not be negative");
   if (rows == 0) return VH_OK;
   if (!x || !block || !y || !rstd || (next_weight && !n)) return set_error(VH_ERR_BAD_ARG, "null pointer");
+  const size_t row = width * elem_size(dtype), all = rows * row;
+  VH_TRY(check_apart({{y, all}, {next_weight ? n : nullptr, all}, {rstd, (size_t)rows * 8, true}},
+                     {{x, all}, {block, all}, {gate, gate_rows * row}, {post_weight, row}, {next_weight, row}}));
   const ResidualNormCall q{x, block, gate, post_weight, next_weight, y, n, rstd, rows, width, gate_rows, scale, eps};
   return VH_DISPATCH(dtype, run_residual_norm, q, S(stream));
 }
@@ -2001,6 +2025,11 @@ int vh_residual_norm_backward(int dtype, const void* grad_y, const void* grad_n,
   }
   if (!x || !block || !rstd || !grad_x || !grad_block || (next_weight ? !grad_n : !grad_y))
     return set_error(VH_ERR_BAD_ARG, "null pointer");
+  const size_t row = width * elem_size(dtype), all = rows * row;
+  VH_TRY(check_apart({{grad_x, all}, {grad_block, all}, {gate ? grad_gate : nullptr, gate_rows * row},
+                      {post_weight ? grad_post_weight : nullptr, row}, {next_weight ? grad_next_weight : nullptr, row}},
+                     {{grad_y, all}, {next_weight ? grad_n : nullptr, all}, {x, all}, {block, all}, {gate, gate_rows * row},
+                      {post_weight, row}, {next_weight, row}, {rstd, (size_t)rows * 8, true}}));
   void* ws;
   VH_TRY(ws_get(st, residual_norm_ws(dtype, rows, width, gate ? gate_rows : 0), &ws));
   const ResidualNormGradCall q{grad_y, grad_n, x, block, gate, post_weight, next_weight, rstd, grad_x, grad_block,
