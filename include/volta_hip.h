@@ -467,14 +467,14 @@ int vh_residual_norm_backward(int dtype, const void* grad_y, const void* grad_n,
  *   A = X X^T,  X <- 3.4445 X + (-4.7750 A + 2.0315 A A) X    `steps` times (1 .. 64; 5 is usual)
  * takes G's singular values to about 1 (0.7 .. 1.2) and keeps its singular vectors; zeros stay zeros, with
  * eps = 0 too.  `grad` and
- * `out` are [batch][rows][cols], batch under 2^22; out may be grad.  VH_F32 is computed to fp32's accuracy; VH_BF16
+ * `out` are [batch][rows][cols], batch under 2^22; out may be grad, or is apart from it.  VH_F32 is computed to fp32's accuracy; VH_BF16
  * with fp16 products and fp32 sums and diagonals, its error below the output's rounding. */
 int vh_orthogonalize(int dtype, const void* grad, void* out, int64_t batch, int64_t rows, int64_t cols, int steps,
                      float eps, void* stream);
 /* One optimiser step on a batch of matrices, in place:
  *   momentum <- beta momentum + grad;  u = nesterov ? grad + beta momentum : momentum
  *   params <- (1 - lr weight_decay) params - lr sqrt(max(1, rows / cols)) orthogonalize(u)
- * params and grads of `dtype`, momentum fp32.  rows / cols is outputs / inputs of a weight that lies
+ * params and grads of `dtype`, momentum fp32 and apart from both.  rows / cols is outputs / inputs of a weight that lies
  * [out][in]; one that lies [in][out], as Linear's, has its factor with lr sqrt(cols / rows) for lr and
  * weight_decay sqrt(rows / cols) for weight_decay. */
 int vh_muon_step(int dtype, void* params, const void* grads, float* momentum, int64_t batch, int64_t rows, int64_t cols,

@@ -2055,6 +2055,8 @@ int vh_orthogonalize(int dtype, const void* grad, void* out, int64_t batch, int6
   VH_TRY(check_orth(dtype, batch, rows, cols, steps, eps));
   if (batch == 0 || rows == 0 || cols == 0) return VH_OK;
   if (!grad || !out) return set_error(VH_ERR_BAD_ARG, "null pointer");
+  const size_t n = (size_t)batch * rows * cols;
+  VH_TRY(check_apart({{out, n * elem_size(dtype)}}, {{grad, n * elem_size(dtype)}}));
   hipStream_t st = S(stream);
   void* ws;
   VH_TRY(ws_get(st, orth_ws(dtype, rows, cols, batch), &ws));
@@ -2068,6 +2070,8 @@ int vh_muon_step(int dtype, void* params, const void* grads, float* momentum, in
   VH_TRY(check_orth(dtype, batch, rows, cols, steps, eps));
   if (batch == 0 || rows == 0 || cols == 0) return VH_OK;
   if (!params || !grads || !momentum) return set_error(VH_ERR_BAD_ARG, "null pointer");
+  const size_t n = (size_t)batch * rows * cols;
+  VH_TRY(check_apart({{params, n * elem_size(dtype)}, {momentum, n * 4, true}}, {{grads, n * elem_size(dtype)}}));
   hipStream_t st = S(stream);
   void* ws;
   VH_TRY(ws_get(st, orth_ws(dtype, rows, cols, batch), &ws));
