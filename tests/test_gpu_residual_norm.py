@@ -313,3 +313,17 @@ def test_refuses_outputs_that_overlap_in_part():
                         (backward, dict(dx=dy, db=dn)), (backward, dict(dx=dy, db=b)), (backward, dict(dwp=wp, dwn=wn, dgate=gate))):
         assert call(**right) == _lib.VH_OK, right
     torch.cuda.synchronize()
+
+
+def test_backward_refuses_other_shapes_of_as_many_elements():
+    """A transposed gradient or rstd would be misread; leading dimensions may be flattened."""
+    t = make(6, 40, torch.float32, 1)
+    y, n, rstd = ops.gpu_residual_norm(t["x"], t["b"], t["gate"], t["wp"], t["wn"])
+    call = lambda dy, dn, r: ops.gpu_residual_norm_backward(dy, dn, t["x"], t["b"], r, t["gate"], t["wp"], t["wn"])  # noqa: E731
+    want = call(t["dy"], t["dn"], rstd)
+    for wrong in ((t["dy"].reshape(40, 6), t["dn"], rstd), (t["dy"], t["dn"].reshape(40, 6), rstd), (t["dy"].reshape(-1), t["dn"], rstd),
+                  (t["dy"], t["dn"], rstd.reshape(6, 2)), (t["dy"], t["dn"], rstd.t().contiguous())):
+        with pytest.raises(volta_amd.VoltaHipError):
+            call(*wrong)
+    got = call(t["dy"].reshape(2, 3, 40), t["dn"].reshape(1, 6, 40), rstd)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -470,10 +470,13 @@ def _residual_norm_backward(x, block, rstd, grad_y, grad_n, gate, post_weight, n
     dt, rows, width, gate_rows = _norm_args(x, block, gate, post_weight, next_weight, what)
     _same_dtype(x, grad_y, grad_n)
     for name, g in (("grad_y", grad_y), ("grad_n", grad_n)):
-        expect_numel(g, rows * width, f"{what} {name}")
+        # leading dimensions may be flattened, rows not
+        if g is not None and (g.numel() != x.numel() or g.dim() < 1 or g.shape[-1] != width):
+            raise VoltaHipError(_lib.VH_ERR_BAD_SHAPE, f"{what} {name}: {tuple(g.shape)}, x is {tuple(x.shape)}")
     if rstd.dtype != torch.float32:
         raise TypeError(f"{what}: rstd is float32")
-    expect_numel(rstd, 2 * rows, f"{what} rstd")
+    if tuple(rstd.shape) != (2, rows):
+        raise VoltaHipError(_lib.VH_ERR_BAD_SHAPE, f"{what} rstd: {tuple(rstd.shape)}, the forward's is {(2, rows)}")
     if next_weight is None and grad_n is not None:
         raise ValueError(f"{what}: grad_n without next_weight")
     new = [torch.empty_like(t) if t is not None else None for t in (x, block, gate, post_weight, next_weight)]
