@@ -469,3 +469,63 @@ def test_logits_and_gradient_beside_each_other(vocab, dtype):
         for p, q in ((a, b), (b, a)):
             with pytest.raises(volta_amd.VoltaHipError):
                 ops.gpu_policy_loss(p, tokens, old, adv, out=q)
+
+
+@pytest.mark.parametrize("vocab", [3, 1000, 16389, 70001, 140001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_policy_loss_alone(vocab, dtype):
+    """Without a gradient: the same loss and log-probabilities, bit for bit."""
+    x, tokens, old, adv, ref = make(5, vocab, dtype, seed=15)
+    mask = torch.tensor([1, 0, 1, 1, 1], dtype=torch.bool, device=DEV)
+    for m in (None, mask):
+        want = ops.gpu_policy_loss(x, tokens, old, adv, ref, m, 0.2, 0.3, 0.1, 0.8, 2.0)
+        loss, logp, grad = ops.gpu_policy_loss(x, tokens, old, adv, ref, m, 0.2, 0.3, 0.1, 0.8, 2.0, grad=False)
+        assert grad is None and torch.equal(loss, want[0]) and torch.equal(logp, want[1])
+        l64, p64 = ref_policy(x, tokens, old, adv, ref, m, 0.2, 0.3, 0.1, 0.8)[:2]
+        assert torch.allclose(logp.double(), p64, rtol=0, atol=8e-6) and abs(float(loss) - float(l64)) <= 2e-5 * max(1.0, abs(float(l64)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [50, 3001, 70001])
+def test_preference_loss_temperature_and_scale(vocab, dtype):
+    """logits / temperature as logits; the gradient by 1 / temperature and by the loss's own."""
+    lens, smooth, beta, temperature, scale = [3, 5, 4, 1], 0.1, 0.3, 1.6, -2.5
+    offsets = torch.tensor([0] + lens, device=DEV).cumsum(0)
+    x, tokens, *_ = make(sum(lens), vocab, dtype, seed=16)
+    cold = x.double() / temperature
+    _, total, _ = ref_preference(cold, tokens, offsets, torch.zeros(4, device=DEV), None, 1.0, 0.0)
+    refs = (total + torch.tensor([1.0, -2.0, 0.5, 0.0], device=DEV)).float()
+    loss, seq, grad = ops.gpu_preference_loss(x, tokens, offsets, refs, None, beta, smooth, temperature, scale)
+    l64, s64, g64 = ref_preference(cold, tokens, offsets, refs, None, beta, smooth)
+    g64 = g64 * (scale / temperature)
+    assert torch.allclose(seq.double(), s64, rtol=1e-6, atol=2e-4) and abs(float(loss) - float(l64)) <= 1e-4
+    tol = 1e-4 * g64.abs().amax(1, keepdim=True) + (2.0 ** -8 * g64.abs() if dtype == torch.bfloat16 else 0)
+    assert float(((grad.double() - g64).abs() - tol).max()) <= 1e-37
+
+
+def test_preference_loss_is_nan_where_the_formula_is():
+    """A NaN, an infinity or a token outside the vocabulary makes its pair's gradients NaN, and the mean; the other
+    pair's, and what a mask leaves out, stay what they are.  Banned entries (-inf) have probability and gradient 0."""
+    clean, tokens, *_ = make(8, 90, torch.float32, seed=17)
+    tokens %= 60
+    clean[:, 80:] = -INF
+    offsets, refs = torch.tensor([0, 2, 4, 6, 8], device=DEV), torch.tensor([-9.0, -8.0, -9.0, -7.0], device=DEV)
+    want = ops.gpu_preference_loss(clean, tokens, offsets, refs)
+    l64, _, g64 = ref_preference(clean, tokens, offsets, refs, None, 0.1, 0.0)
+    assert abs(float(want[0]) - float(l64)) <= 1e-4 and not want[2][:, 80:].any()
+    assert float((want[2].double() - g64).abs().max()) <= 1e-4 * float(g64.abs().max())
+    for value, token in ((float("nan"), None), (INF, None), (None, 90), (None, -1), (None, 1 << 40)):
+        x, tok = clean.clone(), tokens.clone()
+        if token is None:
+            x[1, 5] = value
+        else:
+            tok[1] = token
+        loss, seq, grad = ops.gpu_preference_loss(x, tok, offsets, refs)  # row 1: sequence 0, of pair 0 with sequence 2
+        assert torch.isnan(loss).all() and torch.isnan(seq).tolist() == [True, False, False, False]
+        assert all(bool(torch.isnan(grad[r]).any()) for r in (0, 1, 4, 5))
+        assert torch.equal(grad[[2, 3, 6, 7]], want[2][[2, 3, 6, 7]])
+        mask = torch.ones(8, dtype=torch.bool, device=DEV)
+        mask[1] = False
+        got = ops.gpu_preference_loss(x, tok, offsets, refs, mask)
+        assert all(torch.equal(a, b) for a, b in zip(got, ops.gpu_preference_loss(clean, tokens, offsets, refs, mask)))
+        assert not got[2][1].any()

@@ -327,3 +327,26 @@ def test_backward_refuses_other_shapes_of_as_many_elements():
             call(*wrong)
     got = call(t["dy"].reshape(2, 3, 40), t["dn"].reshape(1, 6, 40), rstd)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("d", [40, 1531, 4096, 9001])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_what_is_not_finite_stays_in_its_row(d, value):
+    """A NaN or an infinity in a row's block, stream or gradient spoils that row and the sums over rows, no other row."""
+    t = make(37, d, torch.float32, 37, seed=4)  # a gate row for each row
+    forward = lambda u: ops.gpu_residual_norm(u["x"], u["b"], u["gate"], u["wp"], u["wn"], 0.5)  # noqa: E731
+    backward = lambda u, r: ops.gpu_residual_norm_backward(u["dy"], u["dn"], u["x"], u["b"], r, u["gate"], u["wp"], u["wn"], 0.5)  # noqa: E731
+    y, n, rstd = forward(t)
+    dx, db, dgate, dwp, dwn = backward(t, rstd)
+    others = torch.arange(37, device=DEV) != 20
+    for name in ("x", "b", "dy", "dn"):
+        u = dict(t, **{name: t[name].clone()})
+        u[name][20, d // 2] = value
+        y2, n2, rstd2 = forward(u)
+        got = backward(u, rstd2)
+        for a, b in zip((y2, n2) + got[:3], (y, n, dx, db, dgate)):
+            assert torch.equal(a[others], b[others]), name
+        if name in ("x", "b"):
+            assert not torch.isfinite(n2[20]).all()
+        assert not torch.isfinite(got[0][20]).all() and not torch.isfinite(got[1][20]).all()
+        assert not torch.isfinite(got[3]).all()
