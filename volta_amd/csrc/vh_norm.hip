@@ -355,8 +355,8 @@ __global__ __launch_bounds__(MOST == 64 ? norm_most_threads(Elem<T>::vec, 64) : 
         if (i * TPR + t < units) {
           const Unit<T> pu = weight(pk, p.wp, 0, i), nu = weight(nk, p.wn, 0, i);
           Unit<T> gu;
-            if constexpr (TOKEN) gu = element(q.g, p.gate, row, i);
-            else gu = weight(gk, p.gate, gate_row, i);
+          if constexpr (TOKEN) gu = element(q.g, p.gate, row, i);
+          else gu = weight(gk, p.gate, gate_row, i);
           Unit<T> o, og, dyu;
           if (p.dy) dyu = element(q.dy, p.dy, row, i);
           float w[VE];
