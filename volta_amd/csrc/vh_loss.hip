@@ -399,10 +399,6 @@ struct PairArgs {
   float beta, smooth;
 };
 
-__device__ __forceinline__ double log1p_exp(double v) {  // log(1 + e^v)
-  return fmax(v, 0.0) + log1p(exp(-fabs(v)));
-}
-
 // One block of two waves per pair: wave 0 sums the chosen sequence, wave 1 the rejected
 // one.  In double, of rows in double: the sums are hundreds or thousands of nats, their
 // difference a few, and fp32 rows of 10 nats were 1e-6 of the loss of 3010 of them.
@@ -421,11 +417,13 @@ __global__ __launch_bounds__(128) void pair_kernel(PairArgs p) {
   __syncthreads();
   if (threadIdx.x) return;
   const double z = (double)p.beta * (sum[0] - sum[1]), e = p.smooth;
-  // an infinite margin (a token of probability 0): a label's share of 0 is none, not 0 infinity
-  p.term[blockIdx.x] = (e < 1 ? (1 - e) * log1p_exp(-z) : 0.0) + (e > 0 ? e * log1p_exp(z) : 0.0);
+  // -log sigmoid(z) = max(-z, 0) + log(1 + t) with t = e^-|z|, and both sigmoids from 1 / (1 + t) and t / (1 + t).
+  // An infinite margin (a token of probability 0): a label's share of 0 is none, not 0 infinity.
+  const double t1 = exp(-fabs(z)), l = log1p(t1), big = 1.0 / (1.0 + t1), small = t1 * big;
+  p.term[blockIdx.x] = (e < 1 ? (1 - e) * (fmax(-z, 0.0) + l) : 0.0) + (e > 0 ? e * (fmax(z, 0.0) + l) : 0.0);
   // e sigmoid(z) - (1 - e) sigmoid(-z): a difference of sigmoid(z) and 1 - e loses what is left of a
   // decided pair's slope (1e-3 of it at z = 30, all of it at 37)
-  const double d = p.beta / p.pairs * (e / (1.0 + exp(-z)) - (1 - e) / (1.0 + exp(z)));
+  const double d = p.beta / p.pairs * (e * (z < 0 ? small : big) - (1 - e) * (z < 0 ? big : small));
   p.coef[blockIdx.x] = (float)d;
   p.coef[blockIdx.x + p.pairs] = (float)-d;
 }
