@@ -665,9 +665,8 @@ constexpr int small_lds(int np) {
   return MP * np * 4 + small_a_bytes<SPLIT, MP, G>() + MP * 8 + 256;
 }
 
-template <bool SPLIT, int MP, int G>
+template <typename T, bool SPLIT, int MP, int G>
 __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32) * G) void orth_small_kernel(SmallArgs p) {
-  using T = std::conditional_t<SPLIT, float, bf16>;
   using ST = typename Elem<T>::storage;
   constexpr int W = MP / 32, WAVES = W * W * G, THREADS = 64 * WAVES, PL = SPLIT ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) char sm[];
@@ -1085,9 +1084,9 @@ int small_rows(long m, long n, int* np) {
   return mp;
 }
 
-template <bool SPLIT, int MP, int G>
+template <typename T, bool SPLIT, int MP, int G>
 int launch_small(const SmallArgs& a, long batch, hipStream_t st) {
-  auto kern = orth_small_kernel<SPLIT, MP, G>;
+  auto kern = orth_small_kernel<T, SPLIT, MP, G>;
   VH_LDS_LIMIT_ONCE(kern);
   kern<<<dim3((unsigned)batch), 64 * (MP / 32) * (MP / 32) * G, small_lds<SPLIT, MP, G>(a.np), st>>>(a);
   VH_LAUNCH_CHECK();
@@ -1157,6 +1156,11 @@ OrthPlan plan_of(long rows, long cols, long batch, bool fp32) {
   o.per_matrix = (o.x_plane + o.a_plane) * 8;
   return o;
 }
+
+// bf16 matrices of fewer elements are computed with both planes, as fp32 ones: the roundings of one plane
+// average over a matrix's entries, and where there are few, were up to 1.7e-2 of a 2 x 3 result, 9e-3 of a
+// number, 6e-3 of 1 x 16 (the largest of 2000; 3.3e-3 at 16 x 16, 2.2e-3 at 128 x 128).  22 us for 18 (16 of 15 x 15).
+constexpr long kFineElems = 256;
 
 constexpr size_t kOrthMostWs = (size_t)1 << 30;
 
@@ -1237,8 +1241,9 @@ int run_orth(const OrthCall& q, char* ws, hipStream_t st) {
     sa.steps = q.steps;
     sa.decay = q.decay;
     sa.step = q.step;
-    if (mp == 128) return launch_small<SPLIT, 128, 1>(sa, q.batch, st);
-    return sa.np == 64 ? launch_small<SPLIT, 64, 1>(sa, q.batch, st) : launch_small<SPLIT, 64, 4>(sa, q.batch, st);
+    if (mp == 128) return launch_small<T, SPLIT, 128, 1>(sa, q.batch, st);
+    if (SPLIT || z >= kFineElems) return sa.np == 64 ? launch_small<T, SPLIT, 64, 1>(sa, q.batch, st) : launch_small<T, SPLIT, 64, 4>(sa, q.batch, st);
+    return sa.np == 64 ? launch_small<T, true, 64, 1>(sa, q.batch, st) : launch_small<T, true, 64, 4>(sa, q.batch, st);
   }
   for (long at = 0; at < q.batch; at += chunk) {
     const long nb = std::min(chunk, q.batch - at);

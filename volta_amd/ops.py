@@ -505,7 +505,7 @@ def gpu_orthogonalize(grad: torch.Tensor, steps: int = 5, eps: float = 1e-7, out
     singular vectors kept.  ``out`` may be ``grad``.
 
     float32 matrices are computed to float32's accuracy; bfloat16 ones with fp16 products and fp32 sums, which over up
-    to 5 steps is off by less than the result's rounding (what is to be more exact goes in as float32)."""
+    to 5 steps is off by about the result's own rounding (what is to be more exact goes in as float32)."""
     what = "gpu_orthogonalize"
     batch, rows, cols = _matrices(grad, what)
     if out is None:
