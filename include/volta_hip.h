@@ -469,8 +469,10 @@ int vh_residual_norm_backward(int dtype, const void* grad_y, const void* grad_n,
  * eps = 0 too.  `grad` and `out` are [batch][rows][cols], batch under 2^22; out may be grad, or is apart
  * from it.  VH_F32 is computed to fp32's accuracy.  VH_BF16 takes fp16 products (one plane of 11 bits of each
  * operand; X by itself to 22) with fp32 sums and diagonals: over up to 5 steps its error is about the output's
- * own rounding (2.0e-3 to 2.4e-3 of the result with it, 1.7e-3 by the rounding alone), every further step adds to
- * it (3e-3 after 10, 1e-2 after 64); matrices of under 256 elements, where it does not average, are computed as VH_F32's.  A caller who wants more of a bf16 matrix passes it as VH_F32. */
+ * own rounding (1.9e-3 to 2.4e-3 of the result with it, up to 3.1e-3 for one or two rows; 1.7e-3 by the rounding
+ * alone), every further step adds to it (3e-3 after 10, 1e-2 after 64).  bf16 matrices of under 4096 elements in
+ * at most 64 rows of 512 (or columns), where it averages less, are computed as VH_F32's; a caller who wants
+ * more of another passes it as VH_F32. */
 int vh_orthogonalize(int dtype, const void* grad, void* out, int64_t batch, int64_t rows, int64_t cols, int steps,
                      float eps, void* stream);
 /* One optimiser step on a batch of matrices, in place:

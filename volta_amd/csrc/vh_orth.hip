@@ -1158,9 +1158,10 @@ OrthPlan plan_of(long rows, long cols, long batch, bool fp32) {
 }
 
 // bf16 matrices of fewer elements are computed with both planes, as fp32 ones: the roundings of one plane
-// average over a matrix's entries, and where there are few, were up to 1.7e-2 of a 2 x 3 result, 9e-3 of a
-// number, 6e-3 of 1 x 16 (the largest of 2000; 3.3e-3 at 16 x 16, 2.2e-3 at 128 x 128).  22 us for 18 (16 of 15 x 15).
-constexpr long kFineElems = 256;
+// average over a matrix's entries, and where there are few, were up to 1.7e-2 of a 2 x 3 result, 3.3e-3 of
+// 16 x 16, 2.7e-3 of 32 x 32 (the largest of 2000; 2.4e-3 at 64 x 64, 2.2e-3 at 128 x 128), of which the output's
+// rounding is 1.7e-3.  It costs 22 us for 18 (16 of 16 x 16), 49 for 39 (of 2 x 500).
+constexpr long kFineElems = 4096;
 
 constexpr size_t kOrthMostWs = (size_t)1 << 30;
 
