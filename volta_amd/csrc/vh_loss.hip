@@ -8,10 +8,10 @@
 // Nothing here multiplies matrices: the passes are bound by memory.  m, s and every
 // sum are fp32 or wider; the gradient is rounded once, to the logits' type.
 //
-// Measured: the policy loss of 2048 rows of 32003 bf16, a quarter masked, in 65 us (3.5 TB/s
+// Measured: the policy loss of 2048 rows of 32003 bf16, a quarter masked, in 64 us (3.5 TB/s
 // read and written), of 4096 rows of 131072 in 435 (4.3); the preference loss of 3010 rows of
 // 50021 in 66 + 6 + 102: its gradient needs every row's log-probability first, so the
-// logits are read a second time (0.3 GB: more than the caches keep); 48 rows of 1000 in 6 + 2.5.
+// logits are read a second time (0.3 GB: more than the caches keep); 48 rows of 1000 in 6 + 2.3.
 //
 // Rows are walked as vh_rows.hpp has it, with 64-bit row offsets: the logits may pass
 // 2^31 elements.

@@ -23,6 +23,7 @@
 //    directions that X lacks grows with the smallest singular values (rank 1: 9e-2
 //    off; 2e-4 so), while B X does not let it through -- if the diagonal of B meets the same
 //    hi as the rest of B does.  bf16 outputs are off by 1.65e-3 for their own rounding.
+//    Small matrices (kFineElems) are computed as fp32 ones.
 #include "vh_kernels.hpp"
 #include "vh_tiles.hpp"
 

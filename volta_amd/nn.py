@@ -294,7 +294,7 @@ def sum_loss_backward(y: torch.Tensor, grad: float = 1.0, out: Optional[torch.Te
 def _on_device(result, what: str):
     """The result of a gpu_* call, whose None (no device path) is an error here."""
     if result is None:
-        raise VoltaHipError(_lib.VH_ERR_NO_DEVICE, f"{what}: the tensors must be on the device")
+        raise VoltaHipError(_lib.VH_ERR_NO_DEVICE, f"{what}: the tensors must be on the device, with memory left for the call")
     return result
 
 
